@@ -33,25 +33,27 @@
 // time.  bf16 contracts over columns in order, 8 (l / 16) + {0..7}, one 16-byte piece of
 // a row; the rows of a state stand for columns accordingly (state_row()).
 //
-// Roundings (bf16): x, y, z enter the matrix cores as they are, P as a sum of two
-// bf16 terms.  Where the result is bf16, the state as an operand is rounded to one
-// (which costs about what the result's own rounding does) and z times its decay is
-// two; where it is float32 (a last state, the decays' gradient) both are three, which
-// hold all 24 bits, so their products are float32's.  The decays' gradient needs r_i
-// . out_i (r the partner of out: q of dq, k of dk): the state's part from the float32
-// accumulators, the chunk's own as sum_j W_ij (x_i . y_j)(r_i . z_j), two products of
-// exact operands.  Sums, states and decays stay in float32, running sums of decays in
-// 64 bits.
+// Roundings (bf16): x, y, z enter the matrix cores as they are; P, z times its decay and
+// the state as an operand each as a sum of two bf16 terms, 2^-16 of them at most.  One
+// term of the state would leave 2^-8 of the part of the result that it carries, which is
+// most of it where decays are slow: 2.2e-3 of the result's norm at decays of 1 - 2^-8,
+// where the result's own rounding is 1.66e-3 (and what is here leaves no more than that).
+// Where the result is float32 (a last state, the decays' gradient) z and the state are
+// three terms, which hold all 24 bits, so their products are float32's.  The decays'
+// gradient needs r_i . out_i (r the partner of out: q of dq, k of dk): the state's part
+// from the float32 accumulators, the chunk's own as sum_j W_ij (x_i . y_j)(r_i . z_j), two
+// products of exact operands.  Sums, states and decays stay in float32, running sums of
+// decays in 64 bits (two float32 terms where weights of P are made from them).
 //
 // What bounds it (MI355X, 4 x 2048 tokens of 16 heads of 128 x 128, bf16; one
-// workgroup of eight waves a CU, 8 chunks each): a pass for o or dv takes 44 us, 151
-// MB of rows and starts at 3.4 TB/s; without its loads and stores 26, without its
-// products 35 (the two overlap in part).  A wave issues 68 matrix instructions of 16
-// cycles a chunk and about 400 vector ones, in phases between two barriers.  A pass
-// with row dots takes 68 us, 124 matrix and 800 vector instructions (the splits into
-// three terms); a summary 26.  A prompt of 32768 tokens of those heads takes 237 us in
-// a row of calls; in a trace its pass is 150 to 160 (3.4 TB/s) and the summary, which
-// reads k and v once more, 85 to 90.
+// workgroup of eight waves a CU, 8 chunks each): a pass for o or dv takes 47 us, 151
+// MB of rows and starts at 3.2 TB/s.  (With one term of the state, 44; then without its
+// loads and stores 26, without its products 35: the two overlap in part.)  A wave issues
+// 84 matrix instructions of 16 cycles a chunk and about 450 vector ones, in phases
+// between two barriers.  A pass with row dots takes 68 us, 124 matrix and 800 vector
+// instructions (the splits into three terms); a summary 26.  A prompt of 32768 tokens of
+// those heads takes 245 us in a row of calls; in a trace, whose launches are longer, its
+// pass is 172 and the summary, which reads k and v once more, 91.
 #pragma once
 
 #include "linear_attention.h"
@@ -196,8 +198,8 @@ __device__ __forceinline__ typename Mat<T>::Frag col_frag(const char* t, uint32_
                  Mat<T>::template column<Tl>(t, at, row0 + 16));
 }
 
-// bf16 terms that P is a sum of: with one, an error of 2^-9 a row of few tokens has in
-// common; with two, the result's own rounding is what counts
+// bf16 terms that P is a sum of: one would be off by up to 2^-8, as much as the result's
+// own rounding; with two, that is what counts
 template <typename T> constexpr int kP = sizeof(T) == 2 ? 2 : 1;
 
 // v as a sum of kN operands (float32: itself)
@@ -680,9 +682,7 @@ __global__ __launch_bounds__(64 * kW, kBuf == 2 || sizeof(T) == 2 ? 2 : kW / 4) 
           f32x4 pij = acc;
           if (jt <= strip) {
             f32x4 d = s_hi[buf][hh][i] - *reinterpret_cast<const f32x4*>(s_hi[buf][hh] + jt * 16 + gq * 4);
-            // the second term matters where results are float32
-            if constexpr (kDot || sizeof(E) == 4)
-              d += s_lo[buf][hh][i] - *reinterpret_cast<const f32x4*>(s_lo[buf][hh] + jt * 16 + gq * 4);
+            d += s_lo[buf][hh][i] - *reinterpret_cast<const f32x4*>(s_lo[buf][hh] + jt * 16 + gq * 4);
 #pragma unroll
             for (int r = 0; r < 4; ++r) pij[r] *= fast_exp2(d[r]) * p_scale;
             if (jt == strip) {

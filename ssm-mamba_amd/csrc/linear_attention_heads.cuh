@@ -183,7 +183,7 @@ __global__ __launch_bounds__(64 * kW, 2) void linear_attention_heads_kernel(cons
         for (int ks = 0; ks < kAS; ++ks)
           acc = M::mma(row_frag<T, TA>(sy + jt * 16 * TA::kRow, row_a, ks), fx[ks], acc);
         f32x4 d = ihi - *reinterpret_cast<const f32x4*>(s_hi[buf] + jt * 16 + gq * 4);
-        if constexpr (kDot) d += ilo - *reinterpret_cast<const f32x4*>(s_lo[buf] + jt * 16 + gq * 4);
+        d += ilo - *reinterpret_cast<const f32x4*>(s_lo[buf] + jt * 16 + gq * 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[r] *= fast_exp2(d[r]) * p_scale;
         if (jt == strip) {
