@@ -181,11 +181,12 @@ LaArgs la_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, co
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// whether a call is to be differentiated
+// whether a call is to be differentiated: backwards, or forwards, which is in force
+// under no_grad too and which the autograd functions refuse
 bool differentiated(std::initializer_list<const at::Tensor*> inputs) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool grad = at::GradMode::is_enabled();
   for (const at::Tensor* t : inputs)
-    if (t->requires_grad()) return true;
+    if ((grad && t->requires_grad()) || t->_fw_grad(0).defined()) return true;
   return false;
 }
 

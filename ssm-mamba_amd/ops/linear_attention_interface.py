@@ -33,7 +33,7 @@ def linear_attention_fn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 
     Rows of adjacent elements that are 16-byte aligned and whole 16 bytes long are
     read in place, whatever their strides; others are copied.  Differentiable once,
-    as ``selective_scan_fn`` is, in q, k, v, g and h_init."""
+    as ``selective_scan_fn`` is, in q, k, v, g and h_init; forward mode is refused."""
     res = _E.module("lm_ops").linear_attention(q, k, v, g, float(scale), h_init, length, padding_side,
                                                bool(return_last_state))
     return (res[0], res[1]) if return_last_state else res[0]
