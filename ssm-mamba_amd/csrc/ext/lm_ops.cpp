@@ -5,6 +5,8 @@
 // embedding's kernels take less time than a Python function of autograd).
 #include "ext_common.h"
 
+#include <torch/csrc/jit/frontend/tracer.h>
+
 #include <algorithm>
 #include <array>
 #include <vector>
@@ -23,6 +25,11 @@ int dtype_code(const at::Tensor& x, const char* name) {
 // written through its address: what autograd saved of it is out of date
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// A trace would hold the results' allocations and not the kernels that fill them.
+void not_traced(const char* name) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), name, " cannot be traced by torch.jit.trace");
 }
 
 // as the step's kernel reads it: any strides, the last one 1
@@ -229,6 +236,7 @@ struct LinearAttentionFn : torch::autograd::Function<LinearAttentionFn> {
 variable_list linear_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                const at::Tensor& g, double scale, const OptT& h_init_, const OptT& length_,
                                const std::string& padding_side, bool want_last) {
+  not_traced("linear_attention_fn");
   check_dim(q, 4, "q");
   check_dim(k, 4, "k");
   check_dim(v, 4, "v");
@@ -258,6 +266,7 @@ variable_list linear_attention(const at::Tensor& q, const at::Tensor& k, const a
 
 at::Tensor linear_attention_step(const at::Tensor& state, const at::Tensor& q_, const at::Tensor& k_,
                                  const at::Tensor& v_, const at::Tensor& g_, double scale) {
+  not_traced("linear_attention_step");
   check_dim(q_, 3, "q");
   check_dim(k_, 3, "k");
   check_dim(v_, 3, "v");
@@ -355,6 +364,7 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
 
 at::Tensor embedding_fn(const at::Tensor& ids, const at::Tensor& weight, double scale,
                         std::optional<int64_t> padding_idx) {
+  not_traced("embedding_fn");
   check_dim(weight, 2, "weight");
   (void)dtype_code(weight, "weight");
   check_ids(ids, weight);
@@ -383,6 +393,7 @@ Range range_of(const at::Tensor& t, size_t owner, bool written) {
 // in place where there are no outs.
 at::Tensor clip_grad_norm(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs,
                           double max_norm) {
+  not_traced("clip_grad_norm_");
   TORCH_CHECK(max_norm >= 0, "max_norm must be >= 0");
   TORCH_CHECK(!grads.empty(), "no gradients");
   const bool inplace = outs.empty();
