@@ -343,6 +343,33 @@ at::Tensor embedding_backward(const at::Tensor& ids_, const at::Tensor& dout_, i
   return dw;
 }
 
+at::Tensor embedding_fn(const at::Tensor& ids, const at::Tensor& weight, double scale,
+                        std::optional<int64_t> padding_idx);
+
+// The weight's gradient as a function of the output's, where that is to be
+// differentiated again: it is linear, with the lookup for its derivative.
+struct EmbeddingGradFn : torch::autograd::Function<EmbeddingGradFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& dout,
+                            int64_t vocab, double scale, int64_t padding_idx) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{vocab, padding_idx};
+    ctx->saved_data["scale"] = scale;
+    return embedding_backward(ids, dout, vocab, scale, padding_idx);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list res(5);
+    if (!grads[0].defined()) return res;
+    const at::Tensor ids = ctx->get_saved_variables()[0];
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const at::Tensor none = ids.lt(0).logical_or(ids.ge(sizes[0])).logical_or(ids.eq(sizes[1]));
+    const auto pad = sizes[1] < 0 ? std::nullopt : std::optional<int64_t>(sizes[1]);
+    res[1] = embedding_fn(ids, grads[0], ctx->saved_data["scale"].toDouble(), pad)
+                 .masked_fill(none.unsqueeze(-1), 0);
+    return res;
+  }
+};
+
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& weight,
                             double scale, int64_t padding_idx) {
@@ -356,8 +383,11 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
-    at::Tensor dw = embedding_backward(ctx->get_saved_variables()[0], plain(grads[0], (at::ScalarType)sizes[1]),
-                                       sizes[0], ctx->saved_data["scale"].toDouble(), sizes[2]);
+    const at::Tensor ids = ctx->get_saved_variables()[0];
+    const at::Tensor dout = plain(grads[0], (at::ScalarType)sizes[1]);
+    const double scale = ctx->saved_data["scale"].toDouble();
+    at::Tensor dw = differentiated({&dout}) ? EmbeddingGradFn::apply(ids, dout, sizes[0], scale, sizes[2])
+                                            : embedding_backward(ids, dout, sizes[0], scale, sizes[2]);
     return {at::Tensor(), dw, at::Tensor(), at::Tensor()};
   }
 };

@@ -16,6 +16,5 @@ def embedding_fn(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     token's rows in float32 in the order of their positions (the same bits every
     time); row ``padding_idx`` gets none, as in ``torch.nn.Embedding``.  A token
     outside the vocabulary gives NaN and no gradient (no exception: the ids stay
-    on the device).  Differentiable once, as ``selective_scan_fn`` is; forward mode is
-    refused."""
+    on the device).  Differentiable any number of times; forward mode is refused."""
     return _E.module("lm_ops").embedding_fn(ids, weight, float(scale), padding_idx)

@@ -32,3 +32,54 @@ def test_forward_mode_of_the_embedding_is_refused(cuda, grad):
     with torch.set_grad_enabled(grad), fwd.dual_level():
         with pytest.raises(RuntimeError, match="jvp is not implemented"):
             embedding_fn(torch.tensor([1, 2], device=cuda), fwd.make_dual(w, torch.ones_like(w)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pad", [None, 3])
+def test_second_and_third_derivatives_of_the_embedding(cuda, dtype, pad):
+    """Whole numbers, exact in every type: against the same formulas by indexing.  The
+    weight's gradient is linear in the output's, so differentiating it gives the lookup
+    (no rows for padding), and that gives the sums again."""
+    from ssm_mamba_amd.ops import embedding_fn
+    vocab, dim = 7, 12
+    gen = torch.Generator().manual_seed(0)
+    ids = torch.randint(0, vocab, (3, 5), generator=gen)
+    whole = lambda *s: torch.randint(-3, 4, s, generator=gen).float()  # noqa: E731
+    w, d, a, b = whole(vocab, dim), whole(3, 5, dim), whole(vocab, dim), whole(3, 5, dim)
+    keep = (ids != pad).float()[..., None] if pad is not None else torch.ones(3, 5, 1)
+    at = ids.to(cuda)
+    W, D, A = (x.to(cuda, dtype).requires_grad_(True) for x in (w, d, a))
+    dw, = torch.autograd.grad(embedding_fn(at, W, scale=2.0, padding_idx=pad), W, D, create_graph=True)
+    sums = lambda x: torch.zeros(vocab, dim).index_add_(0, ids.view(-1), (x * keep).view(-1, dim))  # noqa: E731
+    assert torch.equal(dw.detach().float().cpu(), 2 * sums(d))
+    dd, = torch.autograd.grad(dw, D, A, create_graph=True)
+    assert torch.equal(dd.detach().float().cpu(), 2 * a[ids] * keep)
+    da, = torch.autograd.grad(dd, A, b.to(cuda, dtype))
+    assert torch.equal(da.float().cpu(), 2 * sums(b))
+
+
+def test_second_derivative_through_an_embedding(cuda):
+    """A penalty on the weight's gradient, as a program has it, against torch's."""
+    from ssm_mamba_amd.ops import embedding_fn
+    gen = torch.Generator().manual_seed(1)
+    w0 = torch.randn(11, 8, generator=gen, dtype=torch.float64)
+    ids = torch.randint(0, 11, (20,), generator=gen)
+
+    def penalty(lookup, w):
+        g, = torch.autograd.grad(lookup(w).pow(3).sum(), w, create_graph=True)
+        return torch.autograd.grad(g.square().sum(), w)[0]
+
+    want = penalty(lambda w: w[ids], w0.clone().requires_grad_(True))
+    got = penalty(lambda w: embedding_fn(ids.to(cuda), w), w0.float().to(cuda).requires_grad_(True))
+    # sums of up to 20 products of a few roundings each, twice
+    assert ((got.double().cpu() - want).abs() <= 64 * 2.0 ** -24 * want.abs() + 1e-30).all()
+
+
+def test_tokens_outside_the_vocabulary_twice(cuda):
+    from ssm_mamba_amd.ops import embedding_fn
+    ids = torch.tensor([0, -1, 4, 3], device=cuda)
+    w = torch.ones(4, 8, device=cuda, requires_grad=True)
+    d = torch.ones(4, 8, device=cuda, requires_grad=True)
+    dw, = torch.autograd.grad(embedding_fn(ids, w), w, d, create_graph=True)
+    dd, = torch.autograd.grad(dw.sum(), d)
+    assert torch.equal(dd[:, 0].cpu(), torch.tensor([1.0, 0.0, 0.0, 1.0]))
