@@ -5,6 +5,8 @@
 // embedding's kernels take less time than a Python function of autograd).
 #include "ext_common.h"
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
@@ -197,6 +199,19 @@ bool differentiated(std::initializer_list<const at::Tensor*> inputs) {
   return false;
 }
 
+// The gradients that a backward made with create_graph, `by` those of its results:
+// functions of them and of the node's inputs that raise if differentiated again.
+void once(const char* name, variable_list& grads, const variable_list& by) {
+  using namespace torch::autograd;
+  edge_list from = get_current_node()->next_edges();
+  for (const at::Tensor& t : by)
+    if (t.defined() && t.requires_grad()) from.push_back(impl::gradient_edge(t));
+  const auto error = std::make_shared<Error>(
+      std::string(name) + " is differentiable once: its gradients cannot be differentiated", std::move(from));
+  for (at::Tensor& t : grads)
+    if (t.defined()) impl::set_gradient_edge(t = t.detach(), {error, error->add_input_metadata(t)});
+}
+
 struct LinearAttentionFn : torch::autograd::Function<LinearAttentionFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
                                const at::Tensor& v, const at::Tensor& g, const OptT& h_init,
@@ -229,7 +244,10 @@ struct LinearAttentionFn : torch::autograd::Function<LinearAttentionFn> {
     std::array<bool, 5> need;
     for (int i = 0; i < 5; ++i) need[i] = (i < 4 || a.h_init) && ctx->needs_input_grad(i);
     auto [dq, dk, dv, dg, dh] = la_backward(a, saved[6], saved[7], dout, dlast, need);
-    return {dq, dk, dv, dg, dh, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    variable_list res{dq, dk, dv, dg, dh};
+    if (at::GradMode::is_enabled()) once("linear_attention_fn", res, grads);
+    res.resize(9);
+    return res;
   }
 };
 

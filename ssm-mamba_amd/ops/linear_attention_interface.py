@@ -32,8 +32,9 @@ def linear_attention_fn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
     finite reaches other outputs of its chunk of 64 tokens.
 
     Rows of adjacent elements that are 16-byte aligned and whole 16 bytes long are
-    read in place, whatever their strides; others are copied.  Differentiable once,
-    as ``selective_scan_fn`` is, in q, k, v, g and h_init; forward mode is refused."""
+    read in place, whatever their strides; others are copied.  Differentiable once
+    in q, k, v, g and h_init: differentiating its gradients (create_graph) raises, as
+    forward mode does."""
     res = _E.module("lm_ops").linear_attention(q, k, v, g, float(scale), h_init, length, padding_side,
                                                bool(return_last_state))
     return (res[0], res[1]) if return_last_state else res[0]

@@ -83,3 +83,42 @@ def test_tokens_outside_the_vocabulary_twice(cuda):
     dw, = torch.autograd.grad(embedding_fn(ids, w), w, d, create_graph=True)
     dd, = torch.autograd.grad(dw.sum(), d)
     assert torch.equal(dd[:, 0].cpu(), torch.tensor([1.0, 0.0, 0.0, 1.0]))
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_second_derivatives_of_linear_attention_raise(cuda, shared):
+    """Its gradients themselves may be had with create_graph, as without."""
+    from ssm_mamba_amd.ops import linear_attention_fn
+    x = operands(cuda)
+    if not shared:
+        x["q"], x["k"] = (x[n].repeat_interleave(2, 2) for n in "qk")
+    x = {n: t.requires_grad_(True) for n, t in x.items()}
+    out, last = linear_attention_fn(x["q"], x["k"], x["v"], x["g"], h_init=x["h_init"],
+                                    return_last_state=True)
+    loss = out.square().sum() + last.sum()
+    want = torch.autograd.grad(loss, list(x.values()), retain_graph=True)
+    got = torch.autograd.grad(loss, list(x.values()), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    for g in got:
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="linear_attention_fn is differentiable once"):
+            torch.autograd.grad(g.square().sum(), x["v"], retain_graph=True)
+    # one input's gradient alone, and backward() into .grad
+    only, = torch.autograd.grad(out.sum(), x["k"], retain_graph=True, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        only.sum().backward(retain_graph=True)
+    out.sum().backward()
+    assert all(t.grad is not None and not t.grad.requires_grad for t in x.values())
+
+
+def test_second_derivative_by_the_results_gradient_raises(cuda):
+    """Of operands that are copied on their way, too."""
+    from ssm_mamba_amd.ops import linear_attention_fn
+    x = operands(cuda)
+    wide = torch.randn(1, 70, 2, 17, device=cuda, requires_grad=True)
+    out = linear_attention_fn(wide[..., 1:], x["k"], x["v"], x["g"])
+    d = torch.randn_like(out).requires_grad_(True)
+    dq, = torch.autograd.grad(out, wide, d, create_graph=True)
+    for to in (d, wide):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(dq.sum(), to, retain_graph=True, allow_unused=True)
