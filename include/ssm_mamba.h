@@ -522,7 +522,8 @@ int ssm_decode_pick(int64_t batch, int64_t vocab, int dtype, const void* probs, 
  * 16-byte aligned and are readable to a whole number of 16 bytes (what is past
  * their size is not used; any alignment in a step), tokens key (value) to 2^22
  * elements apart.  heads is a multiple of groups: head h uses query and key head
- * h / (heads / groups).  key, value <= 128.  g: float32 log decays, element (b, t, h) at
+ * h / (heads / groups).  key, value <= 128; batch, heads <= 65535, batch * heads
+ * < 2^23; seqlen < 2^30.  g: float32 log decays, element (b, t, h) at
  * b * g_batch_stride + t * g_token_stride + h (0, 0: one decay per head); -inf
  * clears the state.  h_init, last, dlast, dh_init: (batch, heads, key, value)
  * float32; length, padding_right as in the scan: padded tokens leave the state
@@ -579,8 +580,8 @@ int ssm_linear_attention_step(int64_t batch, int64_t heads, int64_t groups, int6
  * for v = padding_idx (-1: none) and for tokens that do not occur: every row is
  * written.  ids int64 (tokens); weight, dweight (vocab, dim); out, dout
  * (tokens, dim).  A token outside [0, vocab) reads nothing, its output is NaN
- * and it has no gradient.  Sums are float32 in a fixed order.  tokens < 2^31,
- * vocab, dim < 2^30.
+ * and it has no gradient.  Sums are float32 in a fixed order.  tokens <
+ * 2^31 - 65536, vocab, dim < 2^30.
  */
 int ssm_embedding_fwd(int64_t tokens, int64_t vocab, int64_t dim, int dtype, const int64_t* ids,
                       const void* weight, float scale, void* out, void* stream);

@@ -1195,8 +1195,9 @@ int check_la(int64_t batch, int64_t seqlen, int64_t heads, int64_t groups, int64
   if (key > ssm::kLaMaxDim || value > ssm::kLaMaxDim)
     return fail(SSM_ERR_UNSUPPORTED, "linear_attention supports key and value sizes <= %d (got %lld, %lld)",
                 ssm::kLaMaxDim, (long long)key, (long long)value);
-  if (batch > 65535 || heads > 65535 || batch * heads > (1 << 24))
-    return fail(SSM_ERR_UNSUPPORTED, "linear_attention needs batch, heads <= 65535 and batch * heads <= 2^24");
+  // a launch of 512 threads a head holds fewer than 2^32
+  if (batch > 65535 || heads > 65535 || batch * heads >= (1 << 23))
+    return fail(SSM_ERR_UNSUPPORTED, "linear_attention needs batch, heads <= 65535 and batch * heads < 2^23");
   if (seqlen > INT_MAX / 2) return fail(SSM_ERR_UNSUPPORTED, "seqlen must be < 2^30");
   return SSM_OK;
 }

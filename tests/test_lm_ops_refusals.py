@@ -19,3 +19,26 @@ def test_a_trace_is_refused():
             ("clip_grad_norm_", lambda t: clip_grad_norm_(p, 1.0) + t.sum(), w)):
         with pytest.raises(RuntimeError, match=name + " cannot be traced"):
             torch.jit.trace(fn, args)
+
+
+P = 4096  # never dereferenced
+
+
+def test_more_heads_than_a_launch_holds():
+    """512 threads for each of 2^23 heads would be 2^32: refused before any launch."""
+    import ctypes
+
+    from ssm_mamba_amd import _native as N
+    lib = N.lib()
+    b, h = 65535, 129
+    assert b * h >= 1 << 23 and 65535 * 128 < 1 << 23
+    s = (ctypes.c_int64 * 12)(*[4096, 8, 4] * 4)
+    big = 1 << 62
+    got = [lib.ssm_linear_attention_fwd(b, 1, h, 1, 4, 4, 0, P, P, P, s, P, 0, 0, 1.0, None, None, 0, P,
+                                        None, P, P, big, None),
+           lib.ssm_linear_attention_bwd(b, 1, h, 1, 4, 4, 0, P, P, P, P, s, P, 0, 0, 1.0, None, None, 0,
+                                        P, None, None, P, P, P, None, None, P, big, None),
+           lib.ssm_linear_attention_step(b, h, 1, 4, 4, 0, P, P, P, P, s, P, 0, 1.0, P, None)]
+    assert got == [2, 2, 2] and b"batch * heads < 2^23" in lib.ssm_last_error()
+    assert lib.ssm_linear_attention_segments(b, 1, h, 1, 4, 4, 0) == 0
+    assert lib.ssm_linear_attention_segments(65535, 1, 128, 1, 4, 4, 0) == 1
