@@ -436,7 +436,7 @@ struct EmbedPlan {
 EmbedPlan embed_plan(int n, int vocab, int dim) {
   EmbedPlan w{};
   w.per = std::max(kMinPer, ((n + kMaxBlocks - 1) / kMaxBlocks + kThreads - 1) / kThreads * kThreads);
-  w.blocks = (n + w.per - 1) / w.per;
+  w.blocks = (int)(((int64_t)n + w.per - 1) / w.per);
   w.pieces = (n + kPiece - 1) / kPiece;
   size_t at = 0;
   auto take = [&](size_t bytes) {

@@ -42,3 +42,13 @@ def test_more_heads_than_a_launch_holds():
     assert got == [2, 2, 2] and b"batch * heads < 2^23" in lib.ssm_last_error()
     assert lib.ssm_linear_attention_segments(b, 1, h, 1, 4, 4, 0) == 0
     assert lib.ssm_linear_attention_segments(65535, 1, 128, 1, 4, 4, 0) == 1
+
+
+@pytest.mark.parametrize("tokens", [1 << 20, 1 << 29, (1 << 31) - 65537])
+def test_embedding_workspace_of_many_tokens(tokens):
+    """(token, position) pairs twice, 128 workgroups' counts of 1024, a run a row and a
+    row of sums for 32 positions: up to the most tokens there can be."""
+    from ssm_mamba_amd import _native as N
+    got = N.lib().ssm_embedding_bwd_workspace_bytes(tokens, 1000, 2)
+    want = 2 * 8 * tokens + 128 * 1024 * 4 + 1001 * 16 + -(-tokens // 32) * 2 * 4
+    assert want - 128 * 1024 * 4 <= got <= want + 5 * 256
