@@ -35,6 +35,7 @@ constexpr int kMinPer = 512;           // positions a workgroup sorts, at least
 constexpr int kPiece = 32;             // sorted positions summed ahead for long runs
 constexpr int kSmall = 4096;           // positions that one workgroup sorts in one launch
 constexpr int kNoPieces = 1024;        // positions whose runs are summed one by one
+constexpr int kMaxGrid = 1 << 23;      // workgroups of a launch: fewer than 2^32 threads
 
 // ---------------------------------------------------------------- lookup
 
@@ -294,17 +295,17 @@ struct Raw {
   }
 };
 
-// Per piece of kPiece sorted positions: the beginnings and ends of runs in it
-// go to runs[token] (begin, end, first position: a token that occurs once, as most
-// do, needs no more); and a piece that lies inside one run is summed ahead, so
+// Per piece of kPiece sorted positions, from piece `first` on: the beginnings and ends
+// of runs in it go to runs[token] (begin, end, first position: a token that occurs once,
+// as most do, needs no more); and a piece that lies inside one run is summed ahead, so
 // that a frequent token's row adds pieces and not single positions.
 template <typename T, int kE>
 __global__ __launch_bounds__(kThreads) void embed_piece_kernel(const uint2* __restrict__ sorted, int n,
-                                                               int vocab, const T* __restrict__ dout,
+                                                               int first, int vocab, const T* __restrict__ dout,
                                                                int dim, uint4* __restrict__ runs,
                                                                float* __restrict__ part) {
   __shared__ uint32_t s_pos[kPiece];
-  const int lo = blockIdx.x * kPiece, cnt = min(kPiece, n - lo);
+  const int piece = first + blockIdx.x, lo = piece * kPiece, cnt = min(kPiece, n - lo);
   if ((int)threadIdx.x < cnt) {
     const int i = lo + threadIdx.x;
     const uint2 kv = sorted[i];
@@ -327,22 +328,22 @@ __global__ __launch_bounds__(kThreads) void embed_piece_kernel(const uint2* __re
 #pragma unroll
       for (int u = 0; u < 16; ++u) v[u].add(sum);
     }
-    float* o = part + (int64_t)blockIdx.x * dim + c;
+    float* o = part + (int64_t)piece * dim + c;
 #pragma unroll
     for (int e = 0; e < kE; ++e) o[e] = sum[e];
   }
 }
 
-// A workgroup of kX * kY threads takes kY rows of dW; a row's run is single
-// positions up to the first whole piece, pieces, and single positions, kIn of them
-// read at once.
+// A workgroup of kX * kY threads takes kY rows of dW, from row `first` on; a row's run
+// is single positions up to the first whole piece, pieces, and single positions, kIn of
+// them read at once.
 template <typename T, int kE, int kX, int kIn>
 __global__ __launch_bounds__(kThreads) void embed_rows_kernel(const uint2* __restrict__ sorted,
-                                                              const uint4* __restrict__ runs, int vocab,
-                                                              const T* __restrict__ dout, int dim,
+                                                              const uint4* __restrict__ runs, int first,
+                                                              int vocab, const T* __restrict__ dout, int dim,
                                                               const float* __restrict__ part, int pieces,
                                                               float scale, T* __restrict__ dw) {
-  const int row = blockIdx.x * (kThreads / kX) + threadIdx.x / kX;
+  const int row = first + blockIdx.x * (kThreads / kX) + threadIdx.x / kX;
   if (row >= vocab) return;
   const uint4 run = runs[row];
   const int lo = run.x, hi = run.y;
@@ -395,10 +396,11 @@ template <typename T, int kE, int kX>
 void launch_rows(const uint2* sorted, const uint4* runs, int n, int vocab, const T* dout, int dim,
                  const float* part, float scale, T* dw, hipStream_t st) {
   constexpr int kY = kThreads / kX;
-  const dim3 grid((unsigned)((vocab + kY - 1) / kY));
   auto go = [&](auto* kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, sorted, runs, vocab, dout, dim, part,
-                       (int)(n > kNoPieces), scale, dw);
+    const int blocks = (vocab + kY - 1) / kY;
+    for (int k = 0; k < blocks; k += kMaxGrid)
+      hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(blocks - k, kMaxGrid)), dim3(kThreads), 0, st, sorted,
+                         runs, k * kY, vocab, dout, dim, part, (int)(n > kNoPieces), scale, dw);
   };
   // long runs on average: their latency counts; else the registers do
   if (n / vocab >= 8) go(embed_rows_kernel<T, kE, kX, 16>);
@@ -409,9 +411,10 @@ template <typename T, int kE>
 hipError_t launch_sums(const uint2* sorted, uint4* runs, int n, int vocab, const T* dout, int dim,
                        float* part, float scale, T* dw, hipStream_t st) {
   ProfScope prof("embedding_grad", st);
-  if (n > kNoPieces)
-    hipLaunchKernelGGL((embed_piece_kernel<T, kE>), dim3((unsigned)((n + kPiece - 1) / kPiece)),
-                       dim3(kThreads), 0, st, sorted, n, vocab, dout, dim, runs, part);
+  const int parts = n > kNoPieces ? (n + kPiece - 1) / kPiece : 0;
+  for (int k = 0; k < parts; k += kMaxGrid)
+    hipLaunchKernelGGL((embed_piece_kernel<T, kE>), dim3((unsigned)std::min(parts - k, kMaxGrid)),
+                       dim3(kThreads), 0, st, sorted, n, k, vocab, dout, dim, runs, part);
   // a row as wide as the threads that share it
   const int pieces = (dim + kE - 1) / kE;
   if (pieces <= 64) launch_rows<T, kE, 64>(sorted, runs, n, vocab, dout, dim, part, scale, dw, st);
