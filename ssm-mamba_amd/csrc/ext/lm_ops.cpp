@@ -5,6 +5,7 @@
 // embedding's kernels take less time than a Python function of autograd).
 #include "ext_common.h"
 
+#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -476,6 +477,8 @@ at::Tensor clip_grad_norm(const std::vector<at::Tensor>& grads, const std::vecto
     op[i] = dst[i].data_ptr();
     sizes[i] = g.numel();
     if (sizes[i] == 0) continue;
+    TORCH_CHECK(dense || at::has_internal_overlap(o) != at::MemOverlap::Yes,
+                "a gradient that is scaled in place, or an out, has elements that share memory");
     ranges.push_back(range_of(dst[i], i, true));
     if (!inplace && gp[i] != op[i]) ranges.push_back(range_of(src[i], i, false));
   }
