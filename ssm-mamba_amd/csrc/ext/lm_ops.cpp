@@ -456,6 +456,7 @@ at::Tensor clip_grad_norm(const std::vector<at::Tensor>& grads, const std::vecto
   std::vector<int> gt(n), ot(n);
   std::vector<Range> ranges;
   ranges.reserve(2 * n);
+  std::vector<const void*> copied;  // tensors that are written through a copy
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor& g = grads[i];
     TORCH_CHECK(g.layout() == at::kStrided, "gradients must be dense tensors");
@@ -479,10 +480,14 @@ at::Tensor clip_grad_norm(const std::vector<at::Tensor>& grads, const std::vecto
     if (sizes[i] == 0) continue;
     TORCH_CHECK(dense || at::has_internal_overlap(o) != at::MemOverlap::Yes,
                 "a gradient that is scaled in place, or an out, has elements that share memory");
+    if (!dense) copied.push_back(o.data_ptr());
     ranges.push_back(range_of(dst[i], i, true));
     if (!inplace && gp[i] != op[i]) ranges.push_back(range_of(src[i], i, false));
   }
   std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
+  std::sort(copied.begin(), copied.end());
+  TORCH_CHECK(std::adjacent_find(copied.begin(), copied.end()) == copied.end(),
+              "gradients (or outs) overlap: a tensor that is written must be listed once");
   const char* end = nullptr;       // of all ranges so far
   const char* written_end = nullptr;
   for (const Range& r : ranges) {

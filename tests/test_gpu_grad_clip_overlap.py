@@ -35,3 +35,22 @@ def test_elements_that_share_memory(cuda):
         clip_grad_norm_(ps, 0.25, out=[out[0], one.expand(10)])
     torch.cuda.synchronize()
     assert torch.equal(out[0], kept[0]) and float(one) == 2.0
+
+
+@pytest.mark.parametrize("into", [False, True])
+def test_a_strided_tensor_listed_twice(cuda, into):
+    from ssm_mamba_amd.ops import clip_grad_norm_
+    wide = torch.ones(6, 9, device=cuda)
+    if into:
+        ps, out = [param(torch.ones(6, 4, device=cuda)) for _ in "ab"], [wide[:, :4], wide[:, :4]]
+    else:
+        ps, out = [param(wide[:, :4]), param(wide[:, :4])], None
+    with pytest.raises(RuntimeError, match="listed once"):
+        clip_grad_norm_(ps, 0.5, out=out)
+    torch.cuda.synchronize()
+    assert (wide == 1).all()
+    # next to each other in one buffer they are two
+    ps = [param(wide[:, :4]), param(wide[:, 4:])]
+    norm = clip_grad_norm_(ps, 0.5)
+    assert abs(float(norm) - 54 ** 0.5) <= 3 * 2.0 ** -24 * 54 ** 0.5
+    assert (wide < 0.1).all()
