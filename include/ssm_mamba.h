@@ -595,7 +595,9 @@ int ssm_embedding_bwd(int64_t tokens, int64_t vocab, int64_t dim, int dtype, con
  * fixed order) and outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)); the
  * norm stays on the device.  HOST arrays of `count` device pointers, sizes in
  * elements and element types (SSM_F32 or SSM_BF16, an output's its own);
- * outs[i] is grads[i] (in place; both types alike) or overlaps no gradient.
+ * outs[i] is grads[i] (in place; both types alike) or overlaps no gradient.  Fewer
+ * than 2^24 chunks of up to 16384 elements of one gradient; the workspace function
+ * returns 0 for more, and for count < 0 or sizes NULL.
  */
 size_t ssm_grad_clip_workspace_bytes(int64_t count, const int64_t* sizes);
 int ssm_grad_clip(int64_t count, const void* const* grads, void* const* outs, const int64_t* sizes,

@@ -1519,6 +1519,9 @@ int ssm_linear_attention_step(int64_t batch, int64_t heads, int64_t groups, int6
 // ---- embedding and gradient clipping
 namespace {
 
+// workgroups of 256 threads, all in one launch at most: fewer than 2^32 threads
+constexpr int64_t kClipChunks = 1 << 24;
+
 int check_embedding(int64_t tokens, int64_t vocab, int64_t dim, int dtype) {
   if (dtype != SSM_F32 && dtype != SSM_BF16)
     return fail(SSM_ERR_INVALID, "dtype must be SSM_F32 or SSM_BF16 (got %d)", dtype);
@@ -1572,9 +1575,11 @@ int ssm_embedding_bwd(int64_t tokens, int64_t vocab, int64_t dim, int dtype, con
 }
 
 size_t ssm_grad_clip_workspace_bytes(int64_t count, const int64_t* sizes) {
+  if (count < 0 || (count && !sizes)) return 0;
   int64_t chunks = 0;
-  for (int64_t i = 0; i < count; ++i) chunks += sizes[i] > 0 ? ssm::clip_chunks(sizes[i]) : 0;
-  return (size_t)chunks * sizeof(double) + 256;
+  for (int64_t i = 0; i < count && chunks < kClipChunks; ++i)
+    chunks += sizes[i] > 0 ? std::min(ssm::clip_chunks(sizes[i]), kClipChunks) : 0;
+  return chunks < kClipChunks ? (size_t)chunks * sizeof(double) + 256 : 0;
 }
 
 int ssm_grad_clip(int64_t count, const void* const* grads, void* const* outs, const int64_t* sizes,
@@ -1593,9 +1598,10 @@ int ssm_grad_clip(int64_t count, const void* const* grads, void* const* outs, co
         return fail(SSM_ERR_INVALID, "dtype must be SSM_F32 or SSM_BF16 (got %d)", t);
     if (grads[i] == outs[i] && dtypes[i] != out_dtypes[i])
       return fail(SSM_ERR_INVALID, "gradient %lld: in place with another type", (long long)i);
-    chunks += ssm::clip_chunks(sizes[i]);
+    chunks += std::min(ssm::clip_chunks(sizes[i]), kClipChunks);
+    if (chunks >= kClipChunks)
+      return fail(SSM_ERR_UNSUPPORTED, "grad_clip takes fewer than 2^24 chunks of 16384 elements");
   }
-  if (chunks > INT_MAX / 2) return fail(SSM_ERR_UNSUPPORTED, "too many gradient elements");
   if (workspace_bytes < ssm_grad_clip_workspace_bytes(count, sizes))
     return fail(SSM_ERR_INVALID, "grad_clip workspace is %zu bytes, needs %zu", workspace_bytes,
                 ssm_grad_clip_workspace_bytes(count, sizes));

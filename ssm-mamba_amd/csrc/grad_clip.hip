@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void clip_scale_kernel(const ClipTable t,
 
 }  // namespace
 
-int64_t clip_chunks(int64_t n) { return (n + kChunk - 1) / kChunk; }
+int64_t clip_chunks(int64_t n) { return n / kChunk + (n % kChunk != 0); }
 
 // In launches of kClipTensors entries of the list.  ws: a double per chunk and
 // one float.

@@ -52,3 +52,30 @@ def test_embedding_workspace_of_many_tokens(tokens):
     got = N.lib().ssm_embedding_bwd_workspace_bytes(tokens, 1000, 2)
     want = 2 * 8 * tokens + 128 * 1024 * 4 + 1001 * 16 + -(-tokens // 32) * 2 * 4
     assert want - 128 * 1024 * 4 <= got <= want + 5 * 256
+
+
+def test_clipping_more_than_a_launch_holds():
+    """2^24 chunks of 256 threads, sums that would pass 64 bits, and no sizes at all."""
+    import ctypes
+
+    from ssm_mamba_amd import _native as N
+    lib = N.lib()
+    most = (1 << 24) - 1
+
+    def clip(*sizes):
+        n = len(sizes)
+        arr = lambda t, *x: (t * n)(*(x * n if len(x) == 1 else x))  # noqa: E731
+        s = arr(ctypes.c_int64, *sizes)
+        return lib.ssm_grad_clip_workspace_bytes(n, s), lambda: lib.ssm_grad_clip(
+            n, arr(ctypes.c_void_p, P), arr(ctypes.c_void_p, 2 * P), s, arr(ctypes.c_int, 0),
+            arr(ctypes.c_int, 0), 1.0, P, P, 8, None)
+
+    for sizes in ((most * 16384 + 1,), (1 << 37, 1 << 37), ((1 << 63) - 1,),
+                  ((1 << 63) - 1, (1 << 63) - 1, (1 << 63) - 1)):
+        need, call = clip(*sizes)
+        assert need == 0 and call() == 2 and b"2^24 chunks" in lib.ssm_last_error(), sizes
+    need, call = clip(most * 16384)
+    assert need == most * 8 + 256 and call() == 1 and b"workspace" in lib.ssm_last_error()
+    assert lib.ssm_grad_clip_workspace_bytes(-1, None) == 0
+    assert lib.ssm_grad_clip_workspace_bytes(2, None) == 0
+    assert lib.ssm_grad_clip_workspace_bytes(0, None) == 256
