@@ -438,11 +438,51 @@ __device__ __forceinline__ void put_p(char* p, f32x4 v) {
   }
 }
 
-// out^T += Z^T P^T, P's blocks above the diagonal left out
+// 0, or NaN if a value is not finite
+__device__ __forceinline__ float zero_or_nan(f32x4 v) {
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum = fmaf(v[e], 0.f, sum);
+  return sum;
+}
+__device__ __forceinline__ float zero_or_nan(f32x8 v) {
+  return zero_or_nan(__builtin_shufflevector(v, v, 0, 1, 2, 3)) + zero_or_nan(__builtin_shufflevector(v, v, 4, 5, 6, 7));
+}
+__device__ __forceinline__ float zero_or_nan(bf16x8 v) { return zero_or_nan(__builtin_convertvector(v, f32x8)); }
+
+// out^T += Z^T P^T one row of z after the other, to its own row out and later ones
+template <typename T, typename TB, typename TP>
+__device__ __forceinline__ void add_rows(const char* sz, const char* sp, int wave, f32x4 (&out)[4]) {
+  using E = typename Mat<T>::E;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, gq = lane >> 4;
+#pragma unroll 1
+  for (int j = 0; j < kC; ++j) {
+    const f32x4 z = __builtin_convertvector(
+        *reinterpret_cast<const typename Mat<T>::Quad*>(sz + TB::quad(j, wave * 4 + gq)), f32x4);
+    const int jt = j >> 4, jq = j >> 2 & 3;
+    const int u = TP::kHalf ? (jt >> 1) * 8 + jq * 2 + (jt & 1) : jt * 4 + jq;  // as put_p() has it
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int i = it * 16 + l16;
+      if (i < j) continue;
+      const char* const at = sp + TP::quad(i, u) + (j & 3) * sizeof(E);
+      float w = 0.f;
+#pragma unroll
+      for (int k = 0; k < kP<T>; ++k) w += (float)*reinterpret_cast<const E*>(at + k * TP::kBytes);
+      out[it] += w * z;
+    }
+  }
+}
+
+// out^T += Z^T P^T, P's blocks above the diagonal left out.  Inside the others P is zero
+// above it, which is still NaN times a later row of z that is not finite.  The last 16
+// rows out have a product with every row of z: only where one of them is not finite is z
+// looked through, and a chunk with such a value taken row by row.
 template <typename T, typename TB, typename TP>
 __device__ __forceinline__ void add_chunk(const char* sz, const char* sp, uint32_t col_b, uint32_t row_p,
                                           int wave, f32x4 (&out)[4]) {
   using Frag = typename Mat<T>::Frag;
+  const f32x4 before[4] = {out[0], out[1], out[2], out[3]};
 #pragma unroll
   for (int js = 0; js < 2; ++js) {
     const Frag fz = col_frag<T, TB>(sz, TB::quad_tile(col_b, wave), js * 32);
@@ -454,6 +494,16 @@ __device__ __forceinline__ void add_chunk(const char* sz, const char* sp, uint32
         fp[it] = row_frag<T, TP>(sp + k * TP::kBytes + it * 16 * TP::kRow, row_p, js);
 #pragma unroll
       for (int it = 2 * js; it < 4; ++it) out[it] = Mat<T>::mma(fz, fp[it], out[it]);
+    }
+  }
+  if (__any(__builtin_isnan(zero_or_nan(out[3])))) {
+    float z = 0.f;
+#pragma unroll
+    for (int js = 0; js < 2; ++js) z += zero_or_nan(col_frag<T, TB>(sz, TB::quad_tile(col_b, wave), js * 32));
+    if (__any(__builtin_isnan(z))) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it) out[it] = before[it];
+      add_rows<T, TB, TP>(sz, sp, wave, out);
     }
   }
 }

@@ -29,7 +29,7 @@ def linear_attention_fn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 
     bfloat16 results are rounded from float32 sums; the last state, and the
     gradients of g and h_init, are as exact as float32 products.  A value that is not
-    finite reaches other outputs of its chunk of 64 tokens.
+    finite reaches the results that depend on it, and g's gradients at other tokens.
 
     Rows of adjacent elements that are 16-byte aligned and whole 16 bytes long are
     read in place, whatever their strides; others are copied.  Differentiable once
