@@ -1498,7 +1498,6 @@ int ssm_linear_attention_step(int64_t batch, int64_t heads, int64_t groups, int6
   ssm::LaStep p{};
   p.batch = (int)batch;
   p.heads = (int)heads;
-  p.groups = (int)groups;
   p.key = (int)key;
   p.value = (int)value;
   p.state = state;

@@ -16,7 +16,7 @@ struct ClipList {
   const int *dtypes, *out_dtypes;  // 0: float32, 1: bf16
 };
 
-// kClipTensors tensors: tensor i's chunks of kClipChunk elements are the
+// kClipTensors tensors: tensor i's chunks (kChunk elements, grad_clip.hip) are the
 // workgroups first[i] .. first[i + 1] - 1
 struct ClipTable {
   int count;

@@ -46,14 +46,16 @@
 // decays in 64 bits (two float32 terms where weights of P are made from them).
 //
 // What bounds it (MI355X, 4 x 2048 tokens of 16 heads of 128 x 128, bf16; one
-// workgroup of eight waves a CU, 8 chunks each): a pass for o or dv takes 47 us, 151
-// MB of rows and starts at 3.2 TB/s.  (With one term of the state, 44; then without its
+// workgroup of eight waves a CU, 8 chunks each): a pass for o or dv takes 48 us, 151
+// MB of rows and starts at 3.1 TB/s.  (With one term of the state, 44; then without its
 // loads and stores 26, without its products 35: the two overlap in part.)  A wave issues
-// 84 matrix instructions of 16 cycles a chunk and about 450 vector ones, in phases
+// 81 matrix instructions of 16 cycles a chunk and about 530 vector ones, in phases
 // between two barriers.  A pass with row dots takes 68 us, 124 matrix and 800 vector
 // instructions (the splits into three terms); a summary 26.  A prompt of 32768 tokens of
-// those heads takes 245 us in a row of calls; in a trace, whose launches are longer, its
-// pass is 172 and the summary, which reads k and v once more, 91.
+// those heads takes 248 us in a row of calls; in a trace, whose launches are longer, its
+// pass is 184 and the summary, which reads k and v once more, 92.  In float32 it takes
+// 793 (traced 580 and 238): half of the matrix rate, the eight waves' phases are not
+// hidden by another workgroup, for which LDS has no room.
 #pragma once
 
 #include "linear_attention.h"

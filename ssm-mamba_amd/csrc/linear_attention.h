@@ -18,7 +18,7 @@ struct LaTensor {
 };
 
 // One pass out_i = sum_{j <= i} W_ij (x_i . y_j) z_j over one direction of time
-// (see linear_attention.hip).
+// (see linear_attention.cuh).
 struct LaPass {
   int batch, seqlen, heads, seg_len, nseg, reverse;
   int rep;                // heads that share rows
@@ -69,7 +69,7 @@ struct LaDecayGrad {
 };
 
 struct LaStep {
-  int batch, heads, groups, key, value;
+  int batch, heads, key, value;
   float* state;
   LaTensor q, k, v;               // st unused
   const float* g;

@@ -176,8 +176,9 @@ __global__ __launch_bounds__(kThreads) void la_head_sum_kernel(const float* part
 // One token: S <- a S + k v^T, o = scale S^T q.  Pure traffic of the state, so
 // a workgroup takes 4 * kQ columns of one head: kQ lanes with 4 columns each
 // side by side, 256 / kQ rows at a time, and adds the rows' parts of o through
-// LDS.  128 rows of 32 heads of 128 x 64: 54 us, 5.0 TB/s, what a copy reaches; one
-// row of 16 heads of 128 x 128: 5.2 us, the launch.
+// LDS.  128 rows of 32 heads of 128 x 64, 134 MB of states: 54 us from HBM, 5.0 TB/s,
+// what a copy reaches, 42 where the last-level cache still has them; one row of 16
+// heads of 128 x 128: 5.2 us, the launch.
 template <typename T, int kQ, bool kVec>
 __global__ __launch_bounds__(kThreads) void la_step_kernel(const LaStep p, int tiles) {
   constexpr int kRows = kThreads / kQ;

@@ -5,8 +5,10 @@
 // their rows out in the accumulators, so one float32 row leaves for kH heads.  With a
 // workgroup a head that row went out for each: 134 MB written and read again for 4 x
 // 2048 tokens of 32 heads of 128 x 64 over one group, and z and r were read 32
-// times; 95 us and 21 for the sum of the rows, now 87 and 7.  What is left is issue:
-// 16 steps a CU of about 5 us, most of it the splits into three terms.
+// times; 95 us and 21 for the sum of the rows, now 88 and 7.  What is left is issue:
+// 16 steps a CU of about 5 us, most of it the splits into three terms, some of it
+// registers: at 256 of them the compiler spills 38 (108 bytes a lane) and 132 scalar
+// ones into vector ones (64 rows, eight waves, with row dots; up to 99 with four waves).
 //
 // Tiles of x and y are in LDS twice, for this head and the next, those of z and r
 // for this chunk and the next: a head costs one barrier.
@@ -268,8 +270,8 @@ hipError_t launch_heads(const LaPass& p, int blocks, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// kLaHeads heads to a workgroup, whose states are in its registers: as many as a y of
-// 64 rows leaves room for, half of them past that
+// Four heads to a workgroup, whose states are in its registers, where y has up to 64
+// rows, two past that (la_subs())
 template <typename T, int kU, int kO, bool kDot>
 hipError_t launch_heads_dims(const LaPass& p, int blocks, hipStream_t stream) {
   const int a = p.y.dim, b = p.z.dim;
