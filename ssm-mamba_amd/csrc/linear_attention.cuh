@@ -562,7 +562,6 @@ __global__ __launch_bounds__(64 * kW, kBuf == 2 || sizeof(T) == 2 ? 2 : kW / 4) 
   using M = Mat<T>;
   using E = typename M::E;
   using Frag = typename M::Frag;
-  using Quad = typename M::Quad;
   constexpr int kThreads = 64 * kW, kWh = kW / kH, kB = 16 * kWh, kAT = kA / 16, kAS = kA / 32, kBS = kB / 32;
   // float32 products, 16 times as long, are left out where a block is padding
   constexpr bool kSkip = sizeof(E) == 4;

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(64 * kW, 2) void linear_attention_heads_kernel(cons
   const int groups = p.heads / p.rep, grp = unit % groups, b = unit / groups;
   const int h0 = grp * p.rep + sub * kH, nh = min(kH, p.rep - sub * kH);
   const int t0 = seg * p.seg_len, t1 = min(t0 + p.seg_len, p.seqlen);
-  const int nchunks = (t1 - t0 + kC - 1) / kC, nsteps = nchunks * nh;
+  const int nchunks = (t1 - t0 + kC - 1) / kC;
   const int step = p.reverse ? -1 : 1;
   const int ydim = p.y.dim, zdim = p.z.dim;
   const int64_t elems = (int64_t)ydim * zdim;
